@@ -1,0 +1,29 @@
+"""What the measuring tools under tools/ must not do.  CPU only: the sources
+are read, nothing of them is run."""
+import glob
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TOOLS = os.path.join(ROOT, "tools")
+REGISTERS = re.compile(r"\b(?:hip|cuda)HostRegister\s*\(")
+
+
+def sources(*patterns):
+    return sorted(f for p in patterns for f in glob.glob(os.path.join(TOOLS, p)))
+
+
+def text(path):
+    with open(path) as f:
+        return f.read()
+
+
+def test_no_tool_disturbs_a_live_registration():
+    """Five GPU faults of unproven cause followed the registration of memory
+    that the runtime also copied as pageable, or that was freed and used again.
+    No tool brings such a history about: none that registers existing memory
+    copies other parts of it through the runtime, or moves its pages."""
+    disturbs = re.compile(r"MADV_COLLAPSE|torch\.from_numpy")
+    assert sources("*.py")
+    found = [os.path.basename(f) for f in sources("*.py") if REGISTERS.search(text(f)) and disturbs.search(text(f))]
+    assert found == []
