@@ -27,3 +27,10 @@ def test_no_tool_disturbs_a_live_registration():
     assert sources("*.py")
     found = [os.path.basename(f) for f in sources("*.py") if REGISTERS.search(text(f)) and disturbs.search(text(f))]
     assert found == []
+
+
+def test_no_script_registers_existing_memory():
+    """Page-locked memory is allocated (rs_host_alloc, torch's pin_memory);
+    memory that exists already is never registered in place, not for a rate
+    either: every recorded fault followed such a call."""
+    assert [os.path.basename(f) for f in sources("*.py") if REGISTERS.search(text(f))] == []
