@@ -34,3 +34,10 @@ def test_no_script_registers_existing_memory():
     memory that exists already is never registered in place, not for a rate
     either: every recorded fault followed such a call."""
     assert [os.path.basename(f) for f in sources("*.py") if REGISTERS.search(text(f))] == []
+
+
+def test_no_native_tool_registers_existing_memory():
+    """The same for the compiled probes: hipHostMalloc is their only pinned memory."""
+    native = sources("*.hip", "*.cpp", "*.c", "*.hpp")
+    assert native
+    assert [os.path.basename(f) for f in native if REGISTERS.search(text(f))] == []

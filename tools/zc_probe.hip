@@ -5,8 +5,8 @@
 // hipMemcpyAsync calls; the measured time sits ~0.5 ms above the link bound,
 // about 10 us per copy.  A kernel that loads the data shards straight from
 // page-locked host memory and stores the parity straight back has no copies
-// at all and keeps both link directions busy at once.  Legs (all pinned,
-// hipHostMalloc; `reg` = malloc + hipHostRegister, as the JNI path pins):
+// at all and keeps both link directions busy at once.  Legs (all on
+// hipHostMalloc memory, `pin`):
 //   dma_up / dma_down / dma_both   hipMemcpyAsync of the same bytes
 //   zc_read / zc_write             kernel-side loads only / stores only
 //   zc_xor42 (blocks, vec)         4 loads -> 2 stores per column (encode traffic)
@@ -113,82 +113,68 @@ int main(int argc, char **argv) {
     CHECK(hipMalloc(&sink, 256));
     uint8_t *dev = nullptr;
     CHECK(hipMalloc(&dev, 6 * n));
-    for (int mem = 0; mem < 2; ++mem) {
-        uint8_t *h[6];
-        for (int i = 0; i < 6; ++i) {
-            if (mem == 0) {
-                CHECK(hipHostMalloc(reinterpret_cast<void **>(&h[i]), n, hipHostMallocDefault));
-            } else {
-                h[i] = static_cast<uint8_t *>(std::aligned_alloc(4096, n));
-                CHECK(hipHostRegister(h[i], n, hipHostRegisterMapped));
-            }
-            std::memset(h[i], 0x11 * (i + 1), n);
-        }
-        Ptrs p;
-        for (int i = 0; i < 4; ++i) {
-            void *d = nullptr;
-            CHECK(hipHostGetDevicePointer(&d, h[i], 0));
-            p.in[i] = static_cast<const uint8_t *>(d);
-        }
-        for (int i = 0; i < 2; ++i) {
-            void *d = nullptr;
-            CHECK(hipHostGetDevicePointer(&d, h[4 + i], 0));
-            p.out[i] = static_cast<uint8_t *>(d);
-        }
-        const char *mname = mem ? "reg" : "pin";
-        hipStream_t s1, s2;
-        CHECK(hipStreamCreateWithFlags(&s1, hipStreamNonBlocking));
-        CHECK(hipStreamCreateWithFlags(&s2, hipStreamNonBlocking));
-        const double up = 4.0 * n, down = 2.0 * n;
-        report(mname, "dma_up (4 x 64 MiB)", up, 0, median_ms([&] {
-                   for (int i = 0; i < 4; ++i) CHECK(hipMemcpyAsync(dev + i * n, h[i], n, hipMemcpyHostToDevice, 0));
-               }, reps));
-        report(mname, "dma_down (2 x 64 MiB)", 0, down, median_ms([&] {
-                   for (int i = 0; i < 2; ++i) CHECK(hipMemcpyAsync(h[4 + i], dev + (4 + i) * n, n, hipMemcpyDeviceToHost, 0));
-               }, reps));
-        report(mname, "dma_both (two streams)", up, down, median_ms([&] {
-                   hipEvent_t ev;
-                   CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
-                   CHECK(hipEventRecord(ev, 0));
-                   CHECK(hipStreamWaitEvent(s1, ev, 0));
-                   CHECK(hipStreamWaitEvent(s2, ev, 0));
-                   for (int i = 0; i < 4; ++i) CHECK(hipMemcpyAsync(dev + i * n, h[i], n, hipMemcpyHostToDevice, s1));
-                   for (int i = 0; i < 2; ++i) CHECK(hipMemcpyAsync(h[4 + i], dev + (4 + i) * n, n, hipMemcpyDeviceToHost, s2));
-                   hipEvent_t a, b;
-                   CHECK(hipEventCreateWithFlags(&a, hipEventDisableTiming));
-                   CHECK(hipEventCreateWithFlags(&b, hipEventDisableTiming));
-                   CHECK(hipEventRecord(a, s1));
-                   CHECK(hipEventRecord(b, s2));
-                   CHECK(hipStreamWaitEvent(0, a, 0));
-                   CHECK(hipStreamWaitEvent(0, b, 0));
-                   CHECK(hipEventDestroy(a));
-                   CHECK(hipEventDestroy(b));
-                   CHECK(hipEventDestroy(ev));
-               }, reps));
-        const uint64_t nvec = n / 16;
-        for (int blocks : {256, 512, 1024, 2048, 4096}) {
-            char name[64];
-            std::snprintf(name, sizeof name, "zc_read  blocks=%d V=1", blocks);
-            report(mname, name, up, 0, run_zc<1, 1>(p, nvec, sink, blocks, reps));
-            std::snprintf(name, sizeof name, "zc_write blocks=%d V=1", blocks);
-            report(mname, name, 0, down, run_zc<1, 2>(p, nvec, sink, blocks, reps));
-            std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=1", blocks);
-            report(mname, name, up, down, run_zc<1, 0>(p, nvec, sink, blocks, reps));
-            std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=2", blocks);
-            report(mname, name, up, down, run_zc<2, 0>(p, nvec, sink, blocks, reps));
-            std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=4", blocks);
-            report(mname, name, up, down, run_zc<4, 0>(p, nvec, sink, blocks, reps));
-        }
-        CHECK(hipStreamDestroy(s1));
-        CHECK(hipStreamDestroy(s2));
-        for (int i = 0; i < 6; ++i) {
-            if (mem == 0) {
-                CHECK(hipHostFree(h[i]));
-            } else {
-                CHECK(hipHostUnregister(h[i]));
-                std::free(h[i]);
-            }
-        }
+    uint8_t *h[6];
+    for (int i = 0; i < 6; ++i) {
+        CHECK(hipHostMalloc(reinterpret_cast<void **>(&h[i]), n, hipHostMallocDefault));
+        std::memset(h[i], 0x11 * (i + 1), n);
     }
+    Ptrs p;
+    for (int i = 0; i < 4; ++i) {
+        void *d = nullptr;
+        CHECK(hipHostGetDevicePointer(&d, h[i], 0));
+        p.in[i] = static_cast<const uint8_t *>(d);
+    }
+    for (int i = 0; i < 2; ++i) {
+        void *d = nullptr;
+        CHECK(hipHostGetDevicePointer(&d, h[4 + i], 0));
+        p.out[i] = static_cast<uint8_t *>(d);
+    }
+    const char *mname = "pin";
+    hipStream_t s1, s2;
+    CHECK(hipStreamCreateWithFlags(&s1, hipStreamNonBlocking));
+    CHECK(hipStreamCreateWithFlags(&s2, hipStreamNonBlocking));
+    const double up = 4.0 * n, down = 2.0 * n;
+    report(mname, "dma_up (4 x 64 MiB)", up, 0, median_ms([&] {
+               for (int i = 0; i < 4; ++i) CHECK(hipMemcpyAsync(dev + i * n, h[i], n, hipMemcpyHostToDevice, 0));
+           }, reps));
+    report(mname, "dma_down (2 x 64 MiB)", 0, down, median_ms([&] {
+               for (int i = 0; i < 2; ++i) CHECK(hipMemcpyAsync(h[4 + i], dev + (4 + i) * n, n, hipMemcpyDeviceToHost, 0));
+           }, reps));
+    report(mname, "dma_both (two streams)", up, down, median_ms([&] {
+               hipEvent_t ev;
+               CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+               CHECK(hipEventRecord(ev, 0));
+               CHECK(hipStreamWaitEvent(s1, ev, 0));
+               CHECK(hipStreamWaitEvent(s2, ev, 0));
+               for (int i = 0; i < 4; ++i) CHECK(hipMemcpyAsync(dev + i * n, h[i], n, hipMemcpyHostToDevice, s1));
+               for (int i = 0; i < 2; ++i) CHECK(hipMemcpyAsync(h[4 + i], dev + (4 + i) * n, n, hipMemcpyDeviceToHost, s2));
+               hipEvent_t a, b;
+               CHECK(hipEventCreateWithFlags(&a, hipEventDisableTiming));
+               CHECK(hipEventCreateWithFlags(&b, hipEventDisableTiming));
+               CHECK(hipEventRecord(a, s1));
+               CHECK(hipEventRecord(b, s2));
+               CHECK(hipStreamWaitEvent(0, a, 0));
+               CHECK(hipStreamWaitEvent(0, b, 0));
+               CHECK(hipEventDestroy(a));
+               CHECK(hipEventDestroy(b));
+               CHECK(hipEventDestroy(ev));
+           }, reps));
+    const uint64_t nvec = n / 16;
+    for (int blocks : {256, 512, 1024, 2048, 4096}) {
+        char name[64];
+        std::snprintf(name, sizeof name, "zc_read  blocks=%d V=1", blocks);
+        report(mname, name, up, 0, run_zc<1, 1>(p, nvec, sink, blocks, reps));
+        std::snprintf(name, sizeof name, "zc_write blocks=%d V=1", blocks);
+        report(mname, name, 0, down, run_zc<1, 2>(p, nvec, sink, blocks, reps));
+        std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=1", blocks);
+        report(mname, name, up, down, run_zc<1, 0>(p, nvec, sink, blocks, reps));
+        std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=2", blocks);
+        report(mname, name, up, down, run_zc<2, 0>(p, nvec, sink, blocks, reps));
+        std::snprintf(name, sizeof name, "zc_xor42 blocks=%d V=4", blocks);
+        report(mname, name, up, down, run_zc<4, 0>(p, nvec, sink, blocks, reps));
+    }
+    CHECK(hipStreamDestroy(s1));
+    CHECK(hipStreamDestroy(s2));
+    for (int i = 0; i < 6; ++i) CHECK(hipHostFree(h[i]));
     return 0;
 }
