@@ -53,3 +53,10 @@ def test_cpp_tools_compile_against_this_tree():
         p = subprocess.run(["g++", "-std=c++17", "-fsyntax-only", "-D__HIP_PLATFORM_AMD__", "-I", csrc,
                             "-I", os.path.join(rocm, "include"), f], capture_output=True, text=True)
         assert p.returncode == 0, f"{os.path.basename(f)}:\n{p.stderr[:2000]}"
+
+
+def test_runner_leaves_no_progress_of_its_own():
+    """gpu_run.sh's steps show their own progress; a loop beside them would
+    make a hung step look alive."""
+    for f in sources("*.sh"):
+        assert not re.search(r"while\s+(true|:)|heartbeat", text(f)), os.path.basename(f)

@@ -20,10 +20,6 @@ out=gpurun_out
 cd "$GRAFT_REPO_ROOT" || exit 1
 mkdir -p $out
 export TMPDIR=/tmp
-# heartbeat: long legs print nothing for minutes
-(while true; do date +%T > $out/.heartbeat_$tag; sleep 30; done) &
-hb=$!
-trap 'kill $hb 2>/dev/null' EXIT
 np=0
 for step in "$@"; do
   echo "== $step $(date +%T)"
