@@ -93,17 +93,17 @@ int need_device() {
 // because a D2H copy (a blit kernel) queued behind an H2D copy's wait
 // serialises the two directions.  Measured over 0-5 prior streams:
 //   three plain streams                34.3, then 44.0-44.7
-//   D2H / H2D at low / high priority   44.4, 44.4, 44.4, 43.0, 40.6, 42.4
+//   D2H / H2D at low / high priority   44.4, 44.4, 44.4, 43.0, 40.6, 42.4   (no
+//     build has these: work on streams of different priorities can block for good)
 //   three CU-masked streams            43.2-44.4
 //   D2H on the kernel stream           44.1-45.0   <- used
 // The D2H of chunk j now runs before chunk j+1's kernel on one stream, which
 // costs nothing (that kernel waits for its own, longer upload anyway), and
 // only two streams must differ: uploads (stream3) and the rest (stream).
 #ifndef RSAMD_PIPE_MODE
-#define RSAMD_PIPE_MODE 3  // A/B: 0 plain streams, 1 priorities, 2 CU-masked streams, 3 D2H on the kernel stream
+#define RSAMD_PIPE_MODE 3  // A/B: 0 plain streams, 2 CU-masked streams, 3 D2H on the kernel stream
 #endif
 hipError_t create_pipeline_streams(ThreadCtx *c) {
-    int least = 0, greatest = 0;
     if (RSAMD_PIPE_MODE == 2) {
         int dev = 0, ncu = 0;
         hipError_t e = hipGetDevice(&dev);
@@ -114,16 +114,10 @@ hipError_t create_pipeline_streams(ThreadCtx *c) {
         if (e == hipSuccess) e = hipExtStreamCreateWithCUMask(&c->stream3, uint32_t(mask.size()), mask.data());
         return e;
     }
-    if (RSAMD_PIPE_MODE != 1 || hipDeviceGetStreamPriorityRange(&least, &greatest) != hipSuccess || least == greatest) {
-        (void)hipGetLastError();
-        hipError_t e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
-        if (e == hipSuccess) e = hipStreamCreateWithFlags(&c->stream2, hipStreamNonBlocking);
-        if (e == hipSuccess) e = hipStreamCreateWithFlags(&c->stream3, hipStreamNonBlocking);
-        return e;
-    }
+    (void)hipGetLastError();  // an error that the process left behind is not this context's
     hipError_t e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
-    if (e == hipSuccess) e = hipStreamCreateWithPriority(&c->stream2, hipStreamNonBlocking, least);
-    if (e == hipSuccess) e = hipStreamCreateWithPriority(&c->stream3, hipStreamNonBlocking, greatest);
+    if (e == hipSuccess) e = hipStreamCreateWithFlags(&c->stream2, hipStreamNonBlocking);
+    if (e == hipSuccess) e = hipStreamCreateWithFlags(&c->stream3, hipStreamNonBlocking);
     return e;
 }
 
