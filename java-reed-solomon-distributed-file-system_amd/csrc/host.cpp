@@ -1,7 +1,7 @@
 // host.cpp -- the host side of the host-buffer entry points (host.hpp):
-// thread-local error text, per-(thread, device) staging contexts, page-locking
-// of pageable caller buffers, and the chunked H2D -> kernels -> D2H pipeline
-// with its zero-copy path for single-chunk calls.
+// thread-local error text, per-(thread, device) staging contexts, and the
+// chunked H2D -> kernels -> D2H pipeline with its zero-copy path for
+// single-chunk calls.
 #include "host.hpp"
 
 #include <algorithm>

@@ -1,7 +1,7 @@
 // host.hpp -- host side of the C-ABI's host-buffer entry points: error text,
-// the per-(thread, device) staging context, page-locking of caller buffers
-// and the chunked H2D -> kernels -> D2H pipeline (host.cpp).  capi.cpp builds
-// every host-buffer call of include/rs_amd.h on these.
+// the per-(thread, device) staging context and the chunked H2D -> kernels ->
+// D2H pipeline (host.cpp).  capi.cpp builds every host-buffer call of
+// include/rs_amd.h on these.
 #pragma once
 
 #include <hip/hip_runtime.h>
